@@ -10,7 +10,6 @@ one in the low nibble; scales uint8 [pages, kv_heads, page, D / 16], one E4M3 by
 for the whole tensor. Position p of sequence b lives in page table[b, p // page], row p % page.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -24,7 +23,6 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 AXES = {"image": (16, 56, 56), "video": (16, 24, 24), "small": (8, 12, 12), "plane": (32, 32)}
 
 
-@functools.cache
 def _framework():
     folder = str(Path.cwd() / "qwen-image21-tensorfold-rtx_b200")
     if folder not in sys.path:
