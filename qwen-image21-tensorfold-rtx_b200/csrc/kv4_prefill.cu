@@ -662,13 +662,17 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       mma2_ts(kColO + i * 128, i * 128 + 64 + part * 16, b + 4 * 128, id, 1);
     };
     int s = 0, n = 0, nc = 0, both = 0;  // shares so far; the last one's tiles, cached tiles, and if its tile 1 has rows
-    auto advance = [&]() -> bool {       // to the next share with tiles
-      for (n = 0; n == 0; ++s) {
-        const Seg* g = share(s);
-        if (!g) return false;
-        nc = g->nc, n = nc + g->nf, both = g->row0 + 128 < g->rows;
-        share_done(s);
-      }
+    auto take = [&]() -> bool {          // the next share, which may have no tiles; false: none is left
+      const Seg* g = share(s);
+      if (!g) return false;
+      nc = g->nc, n = nc + g->nf, both = g->row0 + 128 < g->rows;
+      share_done(s++);
+      return true;
+    };
+    auto advance = [&]() -> bool {       // to the next share with tiles; only while no results are owed (see below)
+      do {
+        if (!take()) return false;
+      } while (n == 0);
       return true;
     };
     int qs[2] = {0, 0}, ps[2] = {0, 0};  // phases waited for: query rows, probabilities
@@ -679,16 +683,22 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       tc_after();
       qk(i, jj & 1, j < nc);
     };
-    if (advance()) {
-      ok = warp_wait<true>(bar + KFULL, 0, p.err, kErrPrefill + 5);
+    // tile jj of all, the first one of a share, whose keys are waited for here: nothing else is under way
+    auto begin = [&](int jj) {
+      ok = warp_wait<true>(bar + KFULL + (jj & 1), (jj >> 1) & 1, p.err, kErrPrefill + 5);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (ok && i <= both) scores(i, 0, 0);
-      if (ok) mma_commit(bar + KEMPTY);
+        if (ok && i <= both) scores(i, jj, 0);
+      if (ok) mma_commit(bar + KEMPTY + (jj & 1));
+    };
+    if (advance()) {
+      begin(0);
       for (int jj = 0, j = 0; ok; ++jj) {
         const bool last = j + 1 == n, cached = j < nc, add = j > 0;
         const int rows2 = both;
-        const bool more = !last || advance();               // n, nc and both are the next tile's from here on
+        // The next tile is looked for ahead of this one's last product, but only one share ahead: shares without tiles are
+        // handed out behind this share's results (of four shares the block knows at a time), which wait for that product.
+        const bool got = !last || take(), more = got && n > 0;   // n, nc and both are the next tile's from here on
         j = last ? 0 : j + 1;
         ok = warp_wait<true>(bar + VFULL + (jj & 1), (jj >> 1) & 1, p.err, kErrPrefill + 6);
         if (more) ok = ok && warp_wait<true>(bar + KFULL + ((jj + 1) & 1), ((jj + 1) >> 1) & 1, p.err, kErrPrefill + 8);
@@ -711,8 +721,12 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
         }
         if (!ok) break;
         mma_commit(bar + VEMPTY + (jj & 1));
-        if (!more) break;
-        mma_commit(bar + KEMPTY + ((jj + 1) & 1));
+        if (more) {
+          mma_commit(bar + KEMPTY + ((jj + 1) & 1));
+        } else {
+          if (!got || !advance()) break;
+          begin(jj + 1);
+        }
       }
     }
     mma_commit(bar + IDLE);
