@@ -66,6 +66,9 @@ enum Bar {
   GEMPTY = 24
 };
 constexpr int kSegs = 4;                 // row blocks' shares that the warps are told of ahead
+// Some waits last as long as a whole share does (64 million keys a second): the one for room to hand out another, and those
+// of warps that have nothing to do in it. A stall inside a share runs into one of its own waits and ends these as well.
+constexpr long long kShareLimitNs = 60 * kWaitLimitNs;
 
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
 
   // share s of this block's, or null behind the last one (or after an error); each of 21 warps says when it is done with it
   auto share = [&](int s) -> const Seg* {
-    if (!warp_wait(bar + GFULL + s % kSegs, (s / kSegs) & 1, p.err, kErrPrefill + 9)) return nullptr;
+    if (!warp_wait(bar + GFULL + s % kSegs, (s / kSegs) & 1, p.err, kErrPrefill + 9, kShareLimitNs)) return nullptr;
     const Seg* g = seg + s % kSegs;
     return *reinterpret_cast<const volatile int*>(&g->h) < 0 ? nullptr : g;
   };
@@ -445,9 +448,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     bool ok = true;
     // tiles [t0, t1) of a row block, t1 cut to its end; the end of the block's share for at == null
     auto hand_out = [&](const Place* at, int h, int t0, int t1) {
-      // a whole share's time (64 million keys a second), and a stall inside one ends this wait as well
       if (s >= kSegs)
-        ok = ok && warp_wait(bar + GEMPTY + s % kSegs, ((s / kSegs) & 1) ^ 1, p.err, kErrPrefill + 13, 60 * kWaitLimitNs);
+        ok = ok && warp_wait(bar + GEMPTY + s % kSegs, ((s / kSegs) & 1) ^ 1, p.err, kErrPrefill + 13, kShareLimitNs);
       if (!ok) return;
       Seg g;
       g.h = -1;
@@ -807,6 +809,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       const int q_at = row < rows ? row / p.group : g->nq - 1;
       const int see_c = (p.causal && !p.kn ? min(g->len, g->len - g->nq + q_at + 1) : g->len) - g->tile0 * kKeys - half * 64;
       const int see_f = (p.causal ? q_at + 1 : g->nq) - (g->f0 - nc) * kKeys - half * 64;
+      // (a share's first scores, where this query tile had no rows in the one before)
+      if (live) ok = ok && warp_wait(bar + SFULL + i, sp & 1, p.err, kErrPrefill + 10, kShareLimitNs);
       for (int j = 0; live && j < n; ++j) {
         ok = ok && warp_wait(bar + SFULL + i, sp++ & 1, p.err, kErrPrefill + 10);
         if (!ok) {
