@@ -532,6 +532,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     constexpr int CW = D / 32;           // 16-byte pieces of a row's codes
     bool ok = true;
     int sent = -1, done = 0;             // the last tile that TMA was asked for; tiles of the shares so far
+    int made = 0;                        // tiles of all, at the end
     const Seg* g;
     for (int s = 0; ok && (g = share(s)); ++s) {
       const int nc = g->nc, n = nc + g->nf, f0 = g->f0, tile0 = g->tile0, len = g->len, nq = g->nq, h = g->h;
@@ -572,6 +573,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       for (int j = 0; j < nc && ok; ++j) {
         const int jj = done + j, st = jj & 1;
         if (jj >= 2) ok = warp_wait(bar + empty + st, ((jj >> 1) & 1) ^ 1, p.err, kErrPrefill + 1);
+        made = ok ? jj + 1 : jj;
         if (!ok) break;
         uint8_t* tile = ring + st * S::kTileB;
 #pragma unroll
@@ -608,6 +610,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
         for (int j = nc; j < n && ok; ++j) {
           const int jj = done + j, st = jj & 1;
           if (jj >= 2) ok = warp_wait(bar + empty + st, ((jj >> 1) & 1) ^ 1, p.err, kErrPrefill + 4);
+          made = ok ? jj + 1 : jj;
           if (!ok) break;
           const int first = (f0 + j - nc) * kKeys;
           if (mapped && first + kKeys <= nq) {              // whole tiles by TMA: one thread's work
@@ -641,8 +644,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       }
       done += n;
     }
-    // after an error: copies in flight land before the block's shared memory goes away
-    for (int j = max(sent - 1, 0); !ok && j <= sent; ++j) bar_drain(bar + full + (j & 1), (j >> 1) & 1);
+    // Copies in flight land before the block's shared memory goes away, also where an error elsewhere ended the shares or the
+    // products. (Of the last two tiles: a stage that has been filled again was empty before. No wait without an error.)
+    for (int j = max(max(sent - 1, made - 2), 0); j <= sent; ++j) bar_drain(bar + full + (j & 1), (j >> 1) & 1);
   } else if (warp == 20) {
     // ------------------------------------------------------------------------------------------------- products
     const uint32_t qb = smem_u32(smem + S::kQ), kb = smem_u32(smem + S::kK), vb = smem_u32(smem + S::kV);

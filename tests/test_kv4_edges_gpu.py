@@ -1,6 +1,7 @@
 """Edges of attention over the 4-bit cache on the GPU: shares of the work without any keys, lengths that take a block more
 than a second, recorded errors, rows that are not finite, weights spread over many small probabilities. Bounds: tests/_kv4.py."""
 
+import ctypes
 import math
 
 import numpy as np
@@ -9,7 +10,7 @@ import torch
 from _kv4 import attend64, cumulative, ints, make_cache
 from test_kv4_gpu import BF, HF, randn, run_case, takes_many
 
-from tfimage import kv4
+from tfimage import _lib, kv4
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +50,27 @@ def test_a_share_longer_than_a_second(dev, rows):
     got = out.double().cpu().numpy()
     assert (np.abs(got[64:] - ref[64:]) <= tol[64:]).all() and np.isfinite(got).all() and (got[:64] != 0).all()
     assert (np.abs(lse.double().cpu().numpy() - ref_lse) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("rows", [150])
+def test_calls_after_a_recorded_error(dev, rows):
+    """With a code in the device error word (a wait of another kernel that nothing satisfies, as in test_failure_gpu) an
+    attention call returns, whatever its waits find; with the word cleared it gives the bits it gave before."""
+    heads, dim, page = (16, 4), 128, 64
+    cache, table, _ = make_cache(dev, [9000, 3000], heads[1], dim, page, seed=51)
+    lens = ints([9000, 3000], dev)
+    assert takes_many([9000, 3000], [rows, rows], heads, page) == (rows == 150)
+    calls = []
+    for fresh in (False, True):
+        q, k, v = (randn((2 * rows, h, dim), 52 + i, BF).to(dev) for i, h in enumerate((heads[0], heads[1], heads[1])))
+        calls.append(lambda q=q, new=dict(k_new=k, v_new=v) if fresh else {}: kv4.attention(q, cache, table, lens, **new))
+    want = [call() for call in calls]
+    nbytes, _ = _lib.tp_layout(2, 1024, 256)
+    own, silent = (torch.zeros(nbytes, dtype=torch.uint8, device=dev) for _ in range(2))
+    comm = _lib.TpComm(2, 0, (ctypes.c_void_p * _lib.TP_MAX_WORLD)(own.data_ptr(), silent.data_ptr()), 1024, 256)
+    assert _lib.device_status(reset=True) == 0
+    _lib.tp_wait(comm, 1024, 256, 1, dev)
+    for call in calls:
+        call()
+    assert _lib.device_status(reset=True) == 0x304           # the first code stays
+    assert all(torch.equal(call(), w) for call, w in zip(calls, want))
