@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocksPerSm : 2) attn_
   bool ok = true;
   int stage = 0, phase = 0;
   for (int tile = w.tile0 + warp; tile < mid; tile += kWarps) {
-    ok = bar_wait(bars + stage, phase, p.err, kErrDecode);
+    ok = warp_wait(bars + stage, phase, p.err, kErrDecode);   // (shuffles and products of the whole warp follow)
     if (!ok) break;
     const uint8_t* kc = ring + stage * kTileBytes<D>;
     const uint8_t* ks = kc + kTile * (D / 2);

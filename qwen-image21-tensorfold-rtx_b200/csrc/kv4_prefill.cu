@@ -183,12 +183,7 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                      __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// A whole warp's wait (every lane looks: one lane's answer handed round took longer), and its arrival, one for the warp.
-template <bool POLL = false>
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code,
-                                          long long limit = kWaitLimitNs) {
-  return __all_sync(0xffffffffu, bar_wait<POLL>(bar, parity, err, code, limit));
-}
+// A warp's arrival, one for all its lanes.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}"

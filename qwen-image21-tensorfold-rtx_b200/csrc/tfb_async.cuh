@@ -59,6 +59,13 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* er
   const uint32_t a = smem_u32(bar);
   return (POLL ? bar_test(a, parity) : bar_try(a, parity)) || bar_wait_slow<POLL>(a, parity, err, code, limit);
 }
+// A whole warp's wait, with one answer for all lanes: a lane may find the phase complete where another has run out of time or
+// seen an error. (Every lane looks: one lane's answer handed round took longer.)
+template <bool POLL = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code,
+                                          long long limit = kWaitLimitNs) {
+  return __all_sync(0xffffffffu, bar_wait<POLL>(bar, parity, err, code, limit));
+}
 
 // A wait (bounded as well) for what is in flight after an error: it does not stop at the error itself.
 __device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity) {

@@ -52,7 +52,7 @@ def test_a_share_longer_than_a_second(dev, rows):
     assert (np.abs(lse.double().cpu().numpy() - ref_lse) <= tol_lse).all()
 
 
-@pytest.mark.parametrize("rows", [150])
+@pytest.mark.parametrize("rows", [1, 4, 150])
 def test_calls_after_a_recorded_error(dev, rows):
     """With a code in the device error word (a wait of another kernel that nothing satisfies, as in test_failure_gpu) an
     attention call returns, whatever its waits find; with the word cleared it gives the bits it gave before."""
