@@ -31,8 +31,12 @@ struct AttnParams {
                          // their rows' (maximum, sum) pairs
 };
 
-constexpr float kNoMax = -1e30f;   // a row's maximum before its first key: finite, so that exp2(-inf - kNoMax) = 0
-constexpr float kLazy = 8.0f;      // the running maximum follows only a rise by more than 2^8 (fp16 holds 2^15)
+constexpr float kNoMax = -1e30f;   // a row's base before its first key: finite, so that exp2(-inf - kNoMax) = 0
+// A row's powers are taken over a base kHead below its running maximum, which follows only a rise by more than 2^8: at their
+// rounding to 16 bits they reach 2^(kHead + 8) = 2^15 (fp16 holds 65504). So a probability keeps its 11 bits in fp16 down to
+// 2^-21 of the row's largest and is lost below 2^-32 of it, where 262144 keys together weigh 2^-14 (without the head 2^-7).
+constexpr float kHead = 7.0f;
+constexpr float kLazy = 15.0f;     // the base stays while the maximum is at most this far above it
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

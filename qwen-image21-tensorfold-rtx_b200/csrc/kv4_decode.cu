@@ -20,7 +20,8 @@
 //   that the four values of a thread are keys t, 4 + t, 8 + t, 12 + t (shared-memory rows of different banks).
 // A value fragment pairs two keys of one channel: the nibbles of two keys' words are interleaved before the
 // conversion. P^T reaches the second product's layout by movmatrix. E2M1 times its E4M3 scale is exact in fp16; a
-// bf16 query row is brought to fp16 by a power of two (row_exponent). P is rounded to fp16 (2^-11 relative).
+// bf16 query row is brought to fp16 by a power of two (row_exponent). P is rounded to fp16 (by 2^-11 of it or 2^-32 of the
+// row's largest, see kHead), over new keys to q's type.
 #include <math.h>
 
 #include <algorithm>
@@ -66,8 +67,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // Key of row r of a 16-key tile (see the top of the file).
 __device__ __forceinline__ int key_of_row(int r) { return 4 * ((r & 1) + 2 * (r >> 3)) + ((r & 7) >> 1); }
 
-// A warp's state of its 8 * NT query rows: thread (g, t) has rows 2t and 2t + 1 of each 8 in m and l (l: its own share of
-// the sum), and for them channels [g D/8, (g+1) D/8) in o: o[i][n][0], [2] are channels 2i, 2i+1 of row 2t, [1], [3] of
+// A warp's state of its 8 * NT query rows: thread (g, t) has rows 2t and 2t + 1 of each 8 in m (the base of the row's powers)
+// and l (its own share of the sum), and for them channels [g D/8, (g+1) D/8) in o: o[i][n][0], [2] are channels 2i, 2i+1 of row 2t, [1], [3] of
 // row 2t + 1.
 template <int D, int NT>
 struct RowState {
@@ -107,7 +108,7 @@ __device__ __forceinline__ void tile_softmax(RowState<D, NT>& st, float (*s)[NT]
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        const float mn = fmaxf(st.m[n][r], v), c = exp2_fast(st.m[n][r] - mn);
+        const float mn = fmaxf(st.m[n][r], v - kHead), c = exp2_fast(st.m[n][r] - mn);
         st.m[n][r] = mn;
         st.l[n][r] *= c;
 #pragma unroll

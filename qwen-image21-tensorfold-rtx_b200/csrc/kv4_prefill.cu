@@ -11,10 +11,10 @@
 //   warps 0-7, 8-15 : softmax of query tile 0 / 1. Two threads own a row, one for the first 64 keys of a tile, one for the
 //                     others: each reads its scores from TMEM, the two tell one another their maxima (shared memory, a
 //                     barrier of their two warps), and each writes its probabilities back into the scores' columns as the
-//                     packed 16-bit left operand of the second product. The maximum follows only a rise by more than
-//                     2^8; then (seldom) they rescale the accumulator row in TMEM, half of it each. (One thread a row,
-//                     eight warps in all, left an SM's schedulers with two warps that mostly waited for their own
-//                     instructions: 4700 cycles a tile instead of 2048 for its powers.)
+//                     packed 16-bit left operand of the second product. The powers' base follows the maximum only at a
+//                     rise by more than 2^8 (kHead, kLazy); then (seldom) they rescale the accumulator row in TMEM, half
+//                     of it each. (One thread a row, eight warps in all, left an SM's schedulers with two warps that
+//                     mostly waited for their own instructions: 4700 cycles a tile instead of 2048 for its powers.)
 //   warps 16-19     : keys (16, 17) and values (18, 19). Cached tiles: a thread dequantises two rows' codes (E2M1 times E4M3
 //                     is exact in fp16) into shared memory; new tiles: TMA, and 16-byte copies with zeros behind them for
 //                     a sequence's last rows. Keys and values have the same layout (rows of 128 bytes, 128-byte
@@ -28,8 +28,8 @@
 // TMEM: scores of the two query tiles at columns 0 and 128, accumulators at 256 and 384. Products over cached tiles run in
 // fp16 (bf16 query rows brought there by a power of two, see row_exponent), over new tiles in q's type: a softmax thread
 // writes its query row to shared memory, at the border once more, and scales its accumulator by the cache's global value
-// scale. Probabilities are rounded to those types for the second product (2^-11 and, in bf16, 2^-8 relative: as much as the
-// result's own rounding); maxima, sums and accumulators are fp32.
+// scale. Probabilities are rounded to those types for the second product (by 2^-11 and, in bf16, 2^-8 of themselves: as much
+// as the result's own rounding; in fp16 or by 2^-32 of the row's largest); maxima, sums and accumulators are fp32.
 #include <math.h>
 
 #include <algorithm>
@@ -803,7 +803,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       const int row = g->row0 + i * 128 + r, rows = g->rows;
       const int nc = g->nc, nf = g->nf, n = nc + nf;
       const bool live = is_live(g);
-      float m = kNoMax, l = 0.0f;
+      float m = kNoMax, l = 0.0f;                           // base of the powers, their sum
       float mul = nc > 0 ? plain * p.c.k_global * e : plain;
       const int q_at = row < rows ? row / p.group : g->nq - 1;
       const int see_c = (p.causal && !p.kn ? min(g->len, g->len - g->nq + q_at + 1) : g->len) - g->tile0 * kKeys - half * 64;
@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
         mt = fmaxf(mt, tell(mt)) * mul;
         const bool switched = j == nc && j > 0;             // from the cache's value scale to plain values
         if (switched || __any_sync(0xffffffffu, mt > m + kLazy)) {   // (the same in both warps of a row)
-          const float mn = fmaxf(m, mt);
+          const float mn = fmaxf(m, mt - kHead);
           float c = exp2_fast(m - mn);
           m = mn;
           l *= c;

@@ -52,10 +52,11 @@ def cumulative(rows):
     return [0, *np.cumsum(rows).tolist()]
 
 
-def attend64(q, seqs, rows, scale, causal, k_new=None, v_new=None, cached_p=2.0 ** -11, new_p=2.0 ** -8, half_step=2.0 ** -8):
+def attend64(q, seqs, rows, scale, causal, k_new=None, v_new=None, cached_p=2.0 ** -11, new_p=2.0 ** -8, half_step=2.0 ** -8,
+             least_p=2.0 ** -25):
     """float64 attention of packed q [T, Hq, D] (and new rows), and the bound of a kernel's error: half a step of the
     output, half a step of each probability in front of the second product (``cached_p`` / ``new_p``, relative, with
-    2^-25 of the largest for fp16's smallest ones), and fp32 dot products of D terms in the exponent (each score off by
+    ``least_p`` of the largest for fp16's smallest ones), and fp32 dot products of D terms in the exponent (each score off by
     at most (D + 8) 2^-24 sum |q k|, an e-fold as much in the probabilities and their sum; exp2 and the final division
     are within the 8 extra units).
     -> out, lse, bound of out, bound of lse (numpy)."""
@@ -87,7 +88,7 @@ def attend64(q, seqs, rows, scale, causal, k_new=None, v_new=None, cached_p=2.0 
             ds = ds[:, None] + 2.0 ** -22 * (1 + np.abs(top))
             out[lo:lo + n, h] = w @ vh
             spread = w @ np.abs(vh)
-            tiny = 2.0 ** -25 / np.where(some, total, 1.0) * np.abs(vh).sum(0, keepdims=True)
+            tiny = least_p / np.where(some, total, 1.0) * np.abs(vh).sum(0, keepdims=True)
             tol[lo:lo + n, h] = (half_step * np.abs(out[lo:lo + n, h]) + (w * part) @ np.abs(vh) + 2 * np.e * ds * spread
                                  + tiny)
             lse[lo:lo + n, h] = np.where(some, top + np.log(np.where(some, total, 1.0)), -np.inf)[:, 0]

@@ -74,3 +74,35 @@ def test_calls_after_a_recorded_error(dev, rows):
         call()
     assert _lib.device_status(reset=True) == 0x304           # the first code stays
     assert all(torch.equal(call(), w) for call, w in zip(calls, want))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("seqs,rows", [(500, 1), (40, 64)])
+def test_many_small_weights_beside_a_large_one(dev, dtype, seqs, rows):
+    """A key that takes nearly all of the weight and has a value of 0, and 16383 keys of 2^-26.5 of its weight each, whose
+    values have one sign: the result is theirs alone. Probabilities may be lost below 2^-32 of the largest, not before.
+    As many sequences (on the same pages) as leave each to one block, so that the large weight is everyone's base."""
+    heads, dim, page, n = 4, 64, 64, 16384
+    assert takes_many([n] * seqs, [rows] * seqs, (heads, heads), page) == (rows == 64)
+    g = torch.Generator().manual_seed(61)
+    k, v = (torch.randn((n, heads, dim), generator=g) * s for s in (0.25, 0.2))
+    v += 1
+    k[..., 0], k[5], v[5] = 0, 0, 0
+    k[5, :, 0] = 6
+    q = torch.randn((rows, heads, dim), generator=g) * 0.2
+    q[..., 0] = 26.5 * math.log(2) * dim ** 0.5 / 6
+    cache = kv4.Kv4Cache.empty(n // page, page, heads, dim, kv4.global_for(6.0), kv4.global_for(2.0), dev)
+    table = torch.arange(n // page, dtype=torch.int32, device=dev).expand(seqs, -1).contiguous()
+    kv4.write(cache, table[:1], ints([0], dev), k.to(dev), v.to(dev))
+    held = torch.empty((2, n, heads, dim), device=dev)
+    kv4.read(cache, table[:1], ints([0], dev), held[0], held[1])
+    seq = tuple(h.double().cpu().numpy() for h in held)
+    assert (seq[0][5, :, 0] > 5.5).all() and (seq[1][5] == 0).all()
+    q = q.to(dtype)
+    half = torch.finfo(dtype).eps / 2
+    ref, ref_lse, tol, tol_lse = attend64(q.double().numpy(), [seq], [rows], dim ** -0.5, False, half_step=half, least_p=2.0 ** -32)
+    assert (tol / np.abs(ref)).max() < 0.04             # 2^-32 of 16384 keys beside 2^-12.5: 2.2 %, and two roundings of 2^-8
+    out, lse = kv4.attention(q.to(dev).repeat(seqs, 1, 1), cache, table, ints([n] * seqs, dev), return_lse=True)
+    got, e = (t.double().cpu().numpy().reshape(seqs, *r.shape) for t, r in ((out, ref), (lse, ref_lse)))
+    assert (np.abs(got - ref) <= tol).all(), f"worst {np.max(np.abs(got - ref) / tol):.2f} of the bound"
+    assert (np.abs(e - ref_lse) <= tol_lse).all()
