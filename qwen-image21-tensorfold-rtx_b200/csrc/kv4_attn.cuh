@@ -50,6 +50,9 @@ __device__ __forceinline__ int row_exponent(float amax) {
   const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 255u) - 127;
   return amax == 0.0f ? 0 : max(-100, min(100, e));
 }
+// A query row with NaN or an infinity has NaN as its result where it sees a key: its sum starts as NaN, which every
+// sum, factor and logarithm behind it keeps. (Its scores alone would not do: all of them may be -inf.)
+__device__ __forceinline__ float bad_row() { return __uint_as_float(0x7FFFFFFFu); }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 template <typename T>
@@ -250,14 +253,14 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     }
     __syncthreads();
     if (part == 0) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t tok = w.lo + (row0 + row) / p.group;
       const int hq = h * p.group + (row0 + row) % p.group;
       T* dst = static_cast<T*>(p.out) + tok * p.o_st + hq * p.o_sh + lane * V;
 #pragma unroll
       for (int j = 0; j < V; j += 2)
         *reinterpret_cast<uint32_t*>(dst + j) = pack2<T>(acc[j] * inv, acc[j + 1] * inv);
-      if (p.lse && lane == 0) p.lse[tok * p.Hq + hq] = l > 0.0f ? (m + log2f(l)) * 0.69314718056f : -INFINITY;
+      if (p.lse && lane == 0) p.lse[tok * p.Hq + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
     }
   }
 }

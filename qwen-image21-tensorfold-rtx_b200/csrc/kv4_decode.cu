@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocksPerSm : 2) attn_
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = row0 + 8 * n + g;
-    float x[D / 4], amax = 0.0f;
+    float x[D / 4], amax = 0.0f, bad = 0.0f;
     const T* src = static_cast<const T*>(p.q) + (w.lo + r / p.group) * p.q_st + (h * p.group + r % p.group) * p.q_sh +
                    t * (D / 4);
 #pragma unroll
@@ -205,6 +205,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocksPerSm : 2) attn_
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[i + j] = 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) bad = fmaf(x[i], 0.0f, bad);         // NaN if one of them is not finite
+    bad += __shfl_xor_sync(0xffffffffu, bad, 1);
+    bad += __shfl_xor_sync(0xffffffffu, bad, 2);
     int e = 0;
     if (!__is_same(T, __half)) {
 #pragma unroll
@@ -218,7 +222,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocksPerSm : 2) attn_
     for (int i = 0; i < D / 8; ++i) qf[n][i] = pack_f16x2(x[2 * i] * f, x[2 * i + 1] * f);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      mul[n][k] = p.scale_log2 * p.c.k_global * pow2i(__shfl_sync(0xffffffffu, e, (2 * t + k) * 4));
+      const float unit = __shfl_sync(0xffffffffu, bad == 0.0f ? pow2i(e) : bad_row(), (2 * t + k) * 4);
+      mul[n][k] = p.scale_log2 * p.c.k_global * unit;
       const int rr = row0 + 8 * n + 2 * t + k;
       limit[n][k] = p.causal && !p.kn && rr < rows ? min(w.len, w.len - w.nq + rr / p.group + 1) : w.len;
       least = min(least, limit[n][k]);
@@ -234,6 +239,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocksPerSm : 2) attn_
     for (int k = 0; k < 2; ++k) {
       st.m[n][k] = kNoMax;
       st.l[n][k] = 0.0f;
+      if (isnan(mul[n][k]) && (limit[n][k] > 0 || p.kn)) st.l[n][k] = bad_row();
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[i][n][k] = st.o[i][n][2 + k] = 0.0f;
     }
@@ -449,13 +455,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocksPerSm : 2) attn_
       o[4] += f * b.x, o[5] += f * b.y, o[6] += f * b.z, o[7] += f * b.w;
     }
     if (w.nsplit == 1) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] *= inv;
       const int64_t tok = w.lo + row / p.group;
       const int hq = h * p.group + row % p.group;
       store8(static_cast<T*>(p.out) + tok * p.o_st + hq * p.o_sh + c, o);
-      if (p.lse && c == 0) p.lse[tok * p.Hq + hq] = l > 0.0f ? (m + log2f(l)) * 0.69314718056f : -INFINITY;
+      if (p.lse && c == 0) p.lse[tok * p.Hq + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
     } else {
       const int64_t slot = ((int64_t)h * p.items + blockIdx.x) * ROWS + r;
       store8(p.part + slot * D + c, o);

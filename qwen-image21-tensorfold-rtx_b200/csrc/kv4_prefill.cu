@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     };
     auto is_live = [&](const Seg* g) { return g->nc + g->nf > 0 && (i == 0 || g->row0 + 128 < g->rows); };
     // this thread's half of the query row into shared memory, as fp16 over a power of two (`norm`, the result) or as it is;
-    // negated for a negative scale
+    // negated for a negative scale. The result is NaN if a value of it is not finite.
     auto put_query = [&](const Seg* g, bool norm) -> float {
       const int row = g->row0 + i * 128 + r, rows = g->rows;
       const T* src = static_cast<const T*>(p.q) + (g->lo + row / p.group) * p.q_st +
@@ -769,16 +769,18 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
 #pragma unroll
       for (int c = 0; c < D / 16; ++c)
         v[c] = row < rows ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+      using T2 = std::conditional_t<kHalfQ, __half2, __nv_bfloat162>;
+      T2 top2 = __habs2(reinterpret_cast<const T2&>(v[0].x));
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top2 = __hmax2_nan(top2, __habs2(reinterpret_cast<const T2&>(w[k])));
+      }
+      const float lo = __low2float(top2), hi = __high2float(top2), amax = fmaxf(lo, hi);
+      const bool bad = !(lo < INFINITY && hi < INFINITY);
       float e = 1.0f;
       if (norm && !kHalfQ) {
-        float amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          float x[8];
-          unpack_bf16x8(v[c], x);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
-        }
         e = pow2i(row_exponent(fmaxf(amax, tell(amax))));
         const float f = 1.0f / e;
 #pragma unroll
@@ -795,7 +797,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
             make_uint4(v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
       async_fence();
       warp_arrive(bar + QFULL + i);
-      return e;
+      return bad ? bad_row() : e;
     };
     const Seg* g = next_share();
     float e = g && is_live(g) ? put_query(g, g->nc > 0) : 1.0f;
@@ -803,10 +805,12 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       const int row = g->row0 + i * 128 + r, rows = g->rows;
       const int nc = g->nc, nf = g->nf, n = nc + nf;
       const bool live = is_live(g);
-      float m = kNoMax, l = 0.0f;                           // base of the powers, their sum
-      float mul = nc > 0 ? plain * p.c.k_global * e : plain;
       const int q_at = row < rows ? row / p.group : g->nq - 1;
-      const int see_c = (p.causal && !p.kn ? min(g->len, g->len - g->nq + q_at + 1) : g->len) - g->tile0 * kKeys - half * 64;
+      int see_c = p.causal && !p.kn ? min(g->len, g->len - g->nq + q_at + 1) : g->len;
+      float m = kNoMax, l = 0.0f;                           // base of the powers, their sum
+      if (live && isnan(e)) l = see_c > 0 || p.kn ? e : 0.0f, e = 1.0f;
+      float mul = nc > 0 ? plain * p.c.k_global * e : plain;
+      see_c -= g->tile0 * kKeys + half * 64;
       const int see_f = (p.causal ? q_at + 1 : g->nq) - (g->f0 - nc) * kKeys - half * 64;
       // (a share's first scores, where this query tile had no rows in the one before)
       if (live) ok = ok && warp_wait(bar + SFULL + i, sp & 1, p.err, kErrPrefill + 10, kShareLimitNs);
@@ -908,7 +912,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       }
       // ----------------------------------------------------------------------------------------------- results
       const float unit = nf > 0 ? 1.0f : p.c.v_global;      // of the accumulator
-      if (m == kNoMax) l = 0.0f;                            // no key seen (a hidden one's power is 2^-120, not 0)
+      if (m == kNoMax && !isnan(l)) l = 0.0f;               // no key seen (a hidden one's power is 2^-120, not 0)
       const bool part = g->slot >= 0;
       const int64_t tok = g->lo + row / p.group;
       const int hq = g->h * p.group + row % p.group;
@@ -946,7 +950,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
           ml[0] = m;
           ml[1] = l;
         } else if (p.lse) {
-          p.lse[tok * p.Hq + hq] = l > 0.0f ? (m + log2f(l)) * 0.69314718056f : -INFINITY;
+          p.lse[tok * p.Hq + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
         }
       }
       tc_before();
@@ -1033,7 +1037,7 @@ __global__ void __launch_bounds__(256, 4) join_many_kernel(const __grid_constant
       __syncthreads();
     }
     if (of4 == 0 && r < j.rows) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t tok = j.lo + (j.row0 + r) / p.group;
       const int hq = j.h * p.group + (j.row0 + r) % p.group;
       T* dst = static_cast<T*>(p.out) + tok * p.o_st + hq * p.o_sh + eighth * V * 4;
@@ -1042,7 +1046,7 @@ __global__ void __launch_bounds__(256, 4) join_many_kernel(const __grid_constant
         *reinterpret_cast<uint4*>(dst + v * 4) =
             make_uint4(pack2<T>(acc[v].x * inv, acc[v].y * inv), pack2<T>(acc[v].z * inv, acc[v].w * inv),
                        pack2<T>(acc[v + 1].x * inv, acc[v + 1].y * inv), pack2<T>(acc[v + 1].z * inv, acc[v + 1].w * inv));
-      if (p.lse && eighth == 0) p.lse[tok * p.Hq + hq] = l > 0.0f ? (m + log2f(l)) * 0.69314718056f : -INFINITY;
+      if (p.lse && eighth == 0) p.lse[tok * p.Hq + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
     }
   }
 }

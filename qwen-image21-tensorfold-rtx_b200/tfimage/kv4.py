@@ -128,9 +128,10 @@ def attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, lengths: to
     ``k_new`` / ``v_new`` [T, heads, D] (q's type): this call's own keys and values, attended behind the cached ones
     in full precision (they are not written to the cache). ``causal``: with them, row i of a sequence sees its new
     rows up to i; without them the queries are the last rows of the cache, row i of n sees positions up to
-    lengths[b] - n + i. A row that sees nothing gives 0 (and lse -inf). What lies behind a sequence's length is never
-    looked at; rows in front of it must be finite. Row tensors may have any strides with contiguous heads and 16-byte
-    aligned rows. -> out [T, Hq, D], or (out, lse fp32 [T, Hq]: natural logarithm of the row's sum of exponentials)."""
+    lengths[b] - n + i. A row that sees nothing gives 0 (and lse -inf); else a NaN or an infinity in a query row
+    gives NaN (and lse NaN). What lies behind a sequence's length is never looked at; keys and values in front of it must
+    be finite. Row tensors may have any strides with contiguous heads and 16-byte aligned rows.
+    -> out [T, Hq, D], or (out, lse fp32 [T, Hq]: natural logarithm of the row's sum of exponentials)."""
     what = "kv4.attention"
     B, pages, ld = _batch(what, cache, table, lengths, cu)
     dtype, shape = q.dtype, q.shape

@@ -106,3 +106,38 @@ def test_many_small_weights_beside_a_large_one(dev, dtype, seqs, rows):
     got, e = (t.double().cpu().numpy().reshape(seqs, *r.shape) for t, r in ((out, ref), (lse, ref_lse)))
     assert (np.abs(got - ref) <= tol).all(), f"worst {np.max(np.abs(got - ref) / tol):.2f} of the bound"
     assert (np.abs(e - ref_lse) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("lens,rows,heads,causal,fresh", [
+    ([300, 0], [3, 2], (8, 2), False, False), ([3, 700], [5, 9], (4, 4), True, False), ([200, 1], [6, 3], (4, 2), True, True),
+    ([9000], [2], (2, 1), False, False), ([40, 500], [200, 300], (24, 8), True, False), ([0, 2500], [130, 120], (16, 8), False, True),
+    ([3000], [200], (8, 2), False, False), ([1, 0], [1, 260], (32, 32), True, True)])
+def test_query_rows_that_are_not_finite(dev, dtype, lens, rows, heads, causal, fresh):
+    """A NaN or an infinity anywhere in a query row: NaN in its output and lse, or 0 and -inf if it sees nothing. Rows beside it
+    are right."""
+    (Hq, Hk), dim, page = heads, 128, 64
+    cache, table, seqs = make_cache(dev, lens, Hk, dim, page, seed=71, poison=False)
+    T = sum(rows)
+    q = randn((T, Hq, dim), 72, dtype)
+    kn, vn = (randn((T, Hk, dim), 73 + i, dtype) for i in range(2)) if fresh else (None, None)
+    n64 = lambda t: None if t is None else t.double().numpy()   # noqa: E731
+    half = torch.finfo(dtype).eps / 2
+    ref, ref_lse, tol, tol_lse = attend64(n64(q), seqs, rows, dim ** -0.5, causal, n64(kn), n64(vn), new_p=half, half_step=half)
+    bad = torch.zeros((T, Hq), dtype=torch.bool)
+    for i, x in enumerate((float("nan"), float("inf"), -float("inf"))):
+        for j, c in enumerate((0, 37, 64, 127)):
+            r, h = (29 * i + 17 * j) % T, (5 * i + 3 * j) % Hq
+            q[r, h, c] = x
+            bad[r, h] = True
+    q[T - 1, Hq - 1] = float("inf")
+    bad[T - 1, Hq - 1] = True
+    up = lambda t: None if t is None else t.to(dev)   # noqa: E731
+    out, lse = kv4.attention(up(q), cache, table, ints(lens, dev), cu=ints(cumulative(rows), dev), causal=causal, k_new=up(kn),
+                             v_new=up(vn), return_lse=True)
+    got, e, bad = out.double().cpu().numpy(), lse.double().cpu().numpy(), bad.numpy()
+    nothing = np.isneginf(ref_lse)
+    assert np.isnan(got[bad & ~nothing]).all() and np.isnan(e[bad & ~nothing]).all()
+    assert (got[nothing] == 0).all() and np.isneginf(e[nothing]).all()
+    fine = ~bad & ~nothing
+    assert (np.abs(got[fine] - ref[fine]) <= tol[fine]).all() and (np.abs(e[fine] - ref_lse[fine]) <= tol_lse[fine]).all()
