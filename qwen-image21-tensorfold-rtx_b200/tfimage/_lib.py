@@ -339,13 +339,17 @@ class Kv4CacheStruct(ctypes.Structure):
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 
 
+def on_device(index: int, fn, *args):
+    """``fn(*args)`` with CUDA device ``index`` current, whatever device was."""
+    if _current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def launch(index: int, fn, *args) -> None:
     """``fn(*args, stream)`` on CUDA device ``index`` and its current stream, whatever device is current; errors raise."""
-    if _current_device() == index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    status = on_device(index, fn, *args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         check(status)
 

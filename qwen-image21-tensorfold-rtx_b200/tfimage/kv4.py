@@ -151,7 +151,7 @@ def attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, lengths: to
         res = _rows(what, cache, out, T, Hq, dtype)
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     lib = _lib.load()
-    need = lib.tfb_kv4_attention_ws(cache.ref, B, pages, T, Hq)
+    need = _lib.on_device(cache.index, lib.tfb_kv4_attention_ws, cache.ref, B, pages, T, Hq)   # goes by its SMs
     ws = q.new_empty((need,), dtype=torch.uint8) if need > 0 else None
     _lib.launch(cache.index, lib.tfb_kv4_attention, cache.ref, table.data_ptr(), ld, B, pages, lengths.data_ptr(),
                 None if cu is None else cu.data_ptr(), T, Hq, *rows, _lib.OUT_DTYPES[dtype], *new,

@@ -1,0 +1,64 @@
+"""Edges of the 4-bit cache's Python side, without a GPU: the library's calls are taken by a stand-in."""
+
+import contextlib
+
+import pytest
+import torch
+
+from tfimage import _lib, kv4
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it lies on CUDA device 3; nothing here follows its address."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_subclass(cls, t)
+
+    def get_device(self):
+        return 3
+
+    def new_empty(self, *a, **k):
+        return OnGpu(torch.empty(*a, **{"dtype": self.dtype, **k}))
+
+
+def gpu(*shape, dtype=torch.int32):
+    return OnGpu(torch.zeros(shape, dtype=dtype))
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library's calls as (name, device that was current); device 0 is current outside of them."""
+    seen, current = [], [0]
+
+    class Library:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append((name, current[0], args))
+                return 4096 if name.endswith("_ws") else 0
+            return call
+
+    @contextlib.contextmanager
+    def device(index):
+        old, current[0] = current[0], index
+        yield
+        current[0] = old
+
+    monkeypatch.setattr(_lib, "load", lambda: Library())
+    monkeypatch.setattr(_lib, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 1000 + index, raising=False)
+    return seen
+
+
+def cache_on_gpu():
+    new = lambda n: gpu(4, 2, 64, n, dtype=torch.uint8)   # noqa: E731
+    return kv4.Kv4Cache(new(64), new(8), new(64), new(8), 0.01, 0.02)
+
+
+def test_workspace_is_asked_for_on_the_caches_device(calls):
+    """The size goes by the SMs of the device that runs the call, which need not be the current one."""
+    q = gpu(4, 4, 128, dtype=torch.bfloat16)
+    kv4.attention(q, cache_on_gpu(), gpu(2, 3), gpu(2), out=gpu(4, 4, 128, dtype=torch.bfloat16))
+    assert [(name, dev) for name, dev, _ in calls] == [("tfb_kv4_attention_ws", 3), ("tfb_kv4_attention", 3)]
+    assert calls[1][2][-1] == 1003                       # its current stream
