@@ -13,6 +13,7 @@ synchronises, and all three calls can be captured into a CUDA graph and replayed
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -24,29 +25,36 @@ FP4_TOP, E4M3_TOP = 6.0, 448.0
 class Kv4Cache:
     """One layer's cache: codes uint8 [pages, heads, page_size, D / 2] (two E2M1 values a byte, the even one low) and
     scales uint8 [pages, heads, page_size, D / 16] (one E4M3 byte per 16 values) of keys and of values, with one fp32
-    factor each: value = lut[code] * e4m3(scale) * global. page_size: a power of two from 16 to 256; D: 64 or 128."""
+    factor each: value = lut[code] * e4m3(scale) * global. page_size: a power of two from 16 to 256; D: 64 or 128.
 
-    __slots__ = ("k_codes", "k_sf", "v_codes", "v_sf", "k_global", "v_global", "pages", "heads", "page_size", "dim",
-                 "index", "struct", "ref")
+    The calls go by the addresses and factors of the constructor, so they cannot be assigned to: a pool that grows, or
+    gets other factors, is a new Kv4Cache (captured graphs keep the old one's)."""
+
+    __slots__ = ("_k_codes", "_k_sf", "_v_codes", "_v_sf", "_k_global", "_v_global", "_pages", "_heads", "_page_size",
+                 "_dim", "index", "struct", "ref")
 
     def __init__(self, k_codes: torch.Tensor, k_sf: torch.Tensor, v_codes: torch.Tensor, v_sf: torch.Tensor,
                  k_global: float, v_global: float):
         shape = k_codes.shape
         if len(shape) != 4:
             raise _lib.TfbError("Kv4Cache: codes must be [pages, heads, page_size, D / 2]")
-        self.pages, self.heads, self.page_size, half = shape
-        self.dim = 2 * half
-        sf_shape = (self.pages, self.heads, self.page_size, half // 8)
+        self._pages, self._heads, self._page_size, half = shape
+        self._dim = 2 * half
+        sf_shape = (self._pages, self._heads, self._page_size, half // 8)
         self.index, u8 = k_codes.get_device(), torch.uint8
         for t, want in ((k_codes, shape), (v_codes, shape), (k_sf, sf_shape), (v_sf, sf_shape)):
             if t.dtype is not u8 or t.shape != want or not t.is_contiguous() or t.get_device() != self.index:
                 raise _lib.TfbError("Kv4Cache: codes and scales must be contiguous uint8 [pages, heads, page_size, "
                                     "D / 2] and [..., D / 16] on one device")
-        self.k_codes, self.k_sf, self.v_codes, self.v_sf = k_codes, k_sf, v_codes, v_sf
-        self.k_global, self.v_global = k_global, v_global
+        self._k_codes, self._k_sf, self._v_codes, self._v_sf = k_codes, k_sf, v_codes, v_sf
+        self._k_global, self._v_global = k_global, v_global
         self.struct = _lib.Kv4CacheStruct(k_codes.data_ptr(), k_sf.data_ptr(), v_codes.data_ptr(), v_sf.data_ptr(),
-                                          self.pages, self.heads, self.page_size, self.dim, k_global, v_global)
+                                          self._pages, self._heads, self._page_size, self._dim, k_global, v_global)
         self.ref = ctypes.byref(self.struct)
+
+    k_codes, k_sf, v_codes, v_sf, k_global, v_global, pages, heads, page_size, dim = (
+        property(operator.attrgetter("_" + n)) for n in
+        ("k_codes", "k_sf", "v_codes", "v_sf", "k_global", "v_global", "pages", "heads", "page_size", "dim"))
 
     @classmethod
     def empty(cls, pages: int, page_size: int, heads: int, dim: int, k_global: float, v_global: float,
@@ -56,7 +64,7 @@ class Kv4Cache:
         return cls(new(dim // 2), new(dim // 16), new(dim // 2), new(dim // 16), k_global, v_global)
 
     def nbytes(self) -> int:
-        return 2 * (self.k_codes.numel() + self.k_sf.numel())
+        return 2 * (self._k_codes.numel() + self._k_sf.numel())
 
 
 def global_for(amax: float) -> float:
@@ -83,8 +91,8 @@ def _batch(what: str, cache: Kv4Cache, table: torch.Tensor, first: torch.Tensor,
 def _rows(what: str, cache: Kv4Cache, t: torch.Tensor, T: int, heads: int, dtype) -> tuple:
     """(address, row stride, head stride) of rows [T, heads, D]."""
     st = t.stride()
-    if t.shape != (T, heads, cache.dim) or st[2] != 1 or t.dtype is not dtype or t.get_device() != cache.index:
-        raise _lib.TfbError(f"{what}: rows must be {dtype} [{T}, {heads}, {cache.dim}] with contiguous heads on the "
+    if t.shape != (T, heads, cache._dim) or st[2] != 1 or t.dtype is not dtype or t.get_device() != cache.index:
+        raise _lib.TfbError(f"{what}: rows must be {dtype} [{T}, {heads}, {cache._dim}] with contiguous heads on the "
                             f"cache's device (got {t.dtype} {tuple(t.shape)})")
     return t.data_ptr(), st[0], st[1]
 
@@ -96,7 +104,7 @@ def _move(what: str, fn, cache: Kv4Cache, table: torch.Tensor, start: torch.Tens
     if code is None or k.dim() != 3:
         raise _lib.TfbError(f"{what}: k and v must both be bf16, fp16 or fp32 [T, heads, D]")
     T = k.shape[0]
-    kr, vr = _rows(what, cache, k, T, cache.heads, k.dtype), _rows(what, cache, v, T, cache.heads, k.dtype)
+    kr, vr = _rows(what, cache, k, T, cache._heads, k.dtype), _rows(what, cache, v, T, cache._heads, k.dtype)
     _lib.launch(cache.index, fn, cache.ref, table.data_ptr(), ld, B, pages, start.data_ptr(),
                 None if cu is None else cu.data_ptr(), T, *kr, *vr, code)
 
@@ -141,7 +149,7 @@ def attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, lengths: to
     rows = _rows(what, cache, q, T, Hq, dtype)
     new = (None, 0, 0, None, 0, 0)
     if k_new is not None and v_new is not None:
-        new = _rows(what, cache, k_new, T, cache.heads, dtype) + _rows(what, cache, v_new, T, cache.heads, dtype)
+        new = _rows(what, cache, k_new, T, cache._heads, dtype) + _rows(what, cache, v_new, T, cache._heads, dtype)
     elif k_new is not None or v_new is not None:
         raise _lib.TfbError(f"{what}: k_new and v_new go together")
     if out is None:

@@ -62,3 +62,14 @@ def test_workspace_is_asked_for_on_the_caches_device(calls):
     kv4.attention(q, cache_on_gpu(), gpu(2, 3), gpu(2), out=gpu(4, 4, 128, dtype=torch.bfloat16))
     assert [(name, dev) for name, dev, _ in calls] == [("tfb_kv4_attention_ws", 3), ("tfb_kv4_attention", 3)]
     assert calls[1][2][-1] == 1003                       # its current stream
+
+
+@pytest.mark.parametrize("name", ["k_codes", "k_sf", "v_codes", "v_sf", "k_global", "v_global", "pages", "heads", "page_size", "dim"])
+def test_a_cache_cannot_be_changed_behind_its_calls(name):
+    """The calls use the constructor's addresses and factors: assigning others would be silently ignored, or leave them on
+    freed memory."""
+    cache = kv4.Kv4Cache.empty(4, 64, 2, 128, 0.01, 0.02, device="cpu")
+    old = getattr(cache, name)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, torch.cat([old, old]) if isinstance(old, torch.Tensor) else 2 * old)
+    assert getattr(cache, name) is old
