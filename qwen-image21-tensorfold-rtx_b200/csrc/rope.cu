@@ -231,6 +231,7 @@ extern "C" tfb_status tfb_rope_axes(const void* q, void* q_out, int64_t Hq, cons
   if (width > D || (!interleaved && width % 16))
     return fail(TFB_BAD_SHAPE, "rope_axes: the axes' sum (%lld) must be at most the head dim%s", (long long)width,
                 interleaved ? "" : " and a multiple of 16 for half-split pairs");
+  if (B == 0 || N == 0) return TFB_OK;                      // (empty tensors have no address)
   if (!q || !q_out || !ids || (Hk > 0 && (!k || !k_out))) return fail(TFB_BAD_ARG, "rope_axes: null pointer");
   const int item = dtype == TFB_DT_F32 ? 4 : 2;
   const void* ptrs[4] = {q, q_out, k, k_out};
@@ -241,7 +242,6 @@ extern "C" tfb_status tfb_rope_axes(const void* q, void* q_out, int64_t Hq, cons
   }
   if (!aligned(ids, 4) || (wq && !aligned(wq, 4)) || (wk && !aligned(wk, 4)))
     return fail(TFB_BAD_ALIGN, "rope_axes: positions and weights must be 4-byte aligned");
-  if (B == 0 || N == 0) return TFB_OK;
   if (B * N >= (int64_t)1 << 31) return fail(TFB_BAD_SHAPE, "rope_axes: fewer than 2^31 tokens");
   const DeviceInfo* di;
   tfb_status st = device_info(&di);

@@ -1,11 +1,12 @@
 """Edges of the 4-bit cache's Python side, without a GPU: the library's calls are taken by a stand-in."""
 
 import contextlib
+import ctypes
 
 import pytest
 import torch
 
-from tfimage import _lib, kv4
+from tfimage import _lib, kernels as K, kv4
 
 
 class OnGpu(torch.Tensor):
@@ -24,6 +25,18 @@ class OnGpu(torch.Tensor):
 
 def gpu(*shape, dtype=torch.int32):
     return OnGpu(torch.zeros(shape, dtype=dtype))
+
+
+@pytest.mark.parametrize("B,N", [(1, 0), (0, 4), (0, 0)])
+def test_rotation_of_no_tokens(monkeypatch, B, N):
+    """Empty tensors have null addresses."""
+    monkeypatch.setattr(_lib, "launch", lambda index, fn, *args: _lib.check(fn(*args, None)))
+    q, k = (OnGpu(torch.empty((B, N, h, 64), dtype=torch.bfloat16)) for h in (4, 2))
+    out, k_out = K.rope_axes(q, k, OnGpu(torch.empty((N, 3))), (16, 24, 24), q_out=OnGpu(torch.empty_like(q)),
+                             k_out=OnGpu(torch.empty_like(k)))
+    assert out.shape == q.shape and k_out.shape == k.shape
+    assert B or _lib.load().tfb_rope_axes(None, None, 4, None, None, 2, 2, B, 4, 60, (ctypes.c_int64 * 12)(), None, 0, 0, 3, 1,
+                                          (ctypes.c_int * 1)(16), 1e4, None, None, 1e-6, 1, None) == 1   # D is still looked at
 
 
 @pytest.fixture
