@@ -188,7 +188,7 @@ tfb_status check_rows(const char* what, const Kv4Batch& a, const void* k, int64_
     return fail(TFB_BAD_ARG, "%s: unknown element type %d", what, dtype);
   if (!k || !v) return fail(TFB_BAD_ARG, "%s: null pointer", what);
   const int item = dtype == TFB_DT_F32 ? 4 : 2;
-  if (!kv4_rows_aligned(k, k_st, k_sh, item) || !kv4_rows_aligned(v, v_st, v_sh, item))
+  if (!kv4_rows_aligned(k, k_st, k_sh, item, a.T, a.heads) || !kv4_rows_aligned(v, v_st, v_sh, item, a.T, a.heads))
     return fail(TFB_BAD_ALIGN, "%s: k and v must have 16-byte aligned pointers and strides", what);
   if (a.T * a.heads > (int64_t)1 << 34) return fail(TFB_BAD_SHAPE, "%s: more than 2^34 head rows in a call", what);
   return TFB_OK;

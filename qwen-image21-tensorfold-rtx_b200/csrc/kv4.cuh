@@ -70,8 +70,9 @@ inline tfb_status kv4_check(const char* what, const tfb_kv4_cache* c, const int3
   return TFB_OK;
 }
 
-inline bool kv4_rows_aligned(const void* p, int64_t st, int64_t sh, int item) {
-  return aligned(p, 16) && st * item % 16 == 0 && sh * item % 16 == 0;
+// Every head of every row on a 16-byte boundary (the stride of a single row or head is never used).
+inline bool kv4_rows_aligned(const void* p, int64_t st, int64_t sh, int item, int64_t T, int64_t heads) {
+  return aligned(p, 16) && (T == 1 || st * item % 16 == 0) && (heads == 1 || sh * item % 16 == 0);
 }
 
 }  // namespace tfb

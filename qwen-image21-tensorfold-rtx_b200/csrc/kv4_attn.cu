@@ -55,8 +55,9 @@ tfb_status tfb_kv4_attention(const tfb_kv4_cache* c, const int32_t* table, int64
   if (T == 0) return TFB_OK;
   if (!q || !out || (k_new == nullptr) != (v_new == nullptr))
     return fail(TFB_BAD_ARG, "kv4_attention: null pointer (k_new and v_new go together)");
-  if (!kv4_rows_aligned(q, q_st, q_sh, 2) || !kv4_rows_aligned(out, o_st, o_sh, 2) ||
-      (k_new && (!kv4_rows_aligned(k_new, kn_st, kn_sh, 2) || !kv4_rows_aligned(v_new, vn_st, vn_sh, 2))) ||
+  if (!kv4_rows_aligned(q, q_st, q_sh, 2, T, Hq) || !kv4_rows_aligned(out, o_st, o_sh, 2, T, Hq) ||
+      (k_new && (!kv4_rows_aligned(k_new, kn_st, kn_sh, 2, T, c->heads) ||
+                 !kv4_rows_aligned(v_new, vn_st, vn_sh, 2, T, c->heads))) ||
       (lse && !aligned(lse, 4)))
     return fail(TFB_BAD_ALIGN, "kv4_attention: q, out, k_new and v_new must have 16-byte aligned pointers and strides");
   const DeviceInfo* di;

@@ -237,7 +237,8 @@ extern "C" tfb_status tfb_rope_axes(const void* q, void* q_out, int64_t Hq, cons
   const void* ptrs[4] = {q, q_out, k, k_out};
   for (int i = 0; i < (Hk > 0 ? 4 : 2); ++i) {
     bool ok = aligned(ptrs[i], 16);
-    for (int j = 0; j < 3; ++j) ok = ok && strides[3 * i + j] * item % 16 == 0;
+    const int64_t sizes[3] = {B, N, i < 2 ? Hq : Hk};
+    for (int j = 0; j < 3; ++j) ok = ok && (sizes[j] == 1 || strides[3 * i + j] * item % 16 == 0);   // (one: never used)
     if (!ok) return fail(TFB_BAD_ALIGN, "rope_axes: pointers and strides must be 16-byte aligned");
   }
   if (!aligned(ids, 4) || (wq && !aligned(wq, 4)) || (wk && !aligned(wk, 4)))

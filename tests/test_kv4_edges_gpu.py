@@ -10,7 +10,7 @@ import torch
 from _kv4 import attend64, cumulative, ints, make_cache
 from test_kv4_gpu import BF, HF, randn, run_case, takes_many
 
-from tfimage import _lib, kv4
+from tfimage import _lib, kernels as K, kv4
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +141,34 @@ def test_query_rows_that_are_not_finite(dev, dtype, lens, rows, heads, causal, f
     assert (got[nothing] == 0).all() and np.isneginf(e[nothing]).all()
     fine = ~bad & ~nothing
     assert (np.abs(got[fine] - ref[fine]) <= tol[fine]).all() and (np.abs(e[fine] - ref_lse[fine]) <= tol_lse[fine]).all()
+
+
+def test_strides_of_a_single_row_or_head_do_not_matter(dev):
+    """One token out of rows that are not a multiple of 16 bytes long, and one head out of such heads, each on a 16-byte boundary:
+    the same as contiguous ones."""
+    H, D, page = 4, 64, 16
+    cache, table, _ = make_cache(dev, [40], H, D, page, seed=81, poison=False)
+    rows = randn((3, H * D + 4), 82, BF).to(dev)
+    third = lambda t: torch.as_strided(t, (1, H, D), (H * D + 4, D, 1), 2 * (H * D + 4))   # noqa: E731 (520 bytes a row)
+    x = third(rows)
+    assert x.stride(0) % 8 and x.data_ptr() % 16 == 0
+    same = x.contiguous()
+    lens, pos = ints([40], dev), ints([17], dev)
+    want = kv4.attention(same, cache, table, lens, k_new=same, v_new=same)
+    assert torch.equal(kv4.attention(x, cache, table, lens, k_new=x, v_new=x), want)
+    kv4.read(cache, table, pos, back := torch.empty_like(same), torch.empty_like(same))
+    wide = torch.zeros_like(rows)
+    kv4.read(cache, table, pos, third(wide), torch.empty_like(same))
+    assert torch.equal(wide[2, :H * D].view(1, H, D), back) and (wide[:2] == 0).all() and (wide[2, H * D:] == 0).all()
+    kv4.write(cache, table, pos, x, x)
+    kv4.read(cache, table, pos, first := torch.empty_like(same), torch.empty_like(same))
+    kv4.write(cache, table, pos, same, same)
+    kv4.read(cache, table, pos, back, torch.empty_like(same))
+    assert torch.equal(first, back)
+    ids = torch.tensor([[3.0, 4.0, 5.0]], device=dev)
+    want = K.rope_axes(same[None], None, ids, (16, 24, 24))[0]
+    assert torch.equal(K.rope_axes(x[None], None, ids, (16, 24, 24))[0], want)
+    one = torch.as_strided(randn((5, 208), 83, BF).to(dev), (5, 1, D), (208, D + 4, 1), 2 * (D + 4))   # the third of such heads
+    assert one.data_ptr() % 16 == 0 and one.stride(1) % 8
+    assert torch.equal(K.rope_axes(one[None], None, ids.expand(5, 3).contiguous(), (16, 24, 24))[0],
+                       K.rope_axes(one.contiguous()[None], None, ids.expand(5, 3).contiguous(), (16, 24, 24))[0])
