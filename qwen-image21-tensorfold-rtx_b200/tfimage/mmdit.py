@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import itertools
 import math
+import warnings
 from dataclasses import dataclass, field
 
 import torch
@@ -233,7 +234,8 @@ class SynthMMDiT:
         """context [1, L, txt_dim] -> the kept per-block text keys / values (t = 0 modulation, causal). ``into``: an
         earlier prefix of the same length whose buffers are overwritten (captured step graphs keep using them).
         ``cache="nvfp4"``: keys and values are kept in 4 bits (9/16 byte a value instead of 2), quantised under global
-        scales that leave ``CACHE_MARGIN`` times this prompt's largest values (``into`` keeps its scales)."""
+        scales that leave ``CACHE_MARGIN`` times this prompt's largest values (``into`` keeps its scales, and warns
+        of a prompt whose values pass them and saturate)."""
         cfg = self.cfg
         c = context.to(self.device).float()
         c = c * torch.rsqrt(c.pow(2).mean(-1, keepdim=True) + cfg.eps) * self.txt_norm
@@ -266,14 +268,22 @@ class SynthMMDiT:
     def _keep_in_4_bits(self, kv: list, prefix: Prefix | None, B: int, P: int) -> Prefix:
         """The blocks' (k, v) [B, P, H, D] into 4-bit caches: new ones, or those of an earlier ``prefix``."""
         cfg = self.cfg
+        tops = None
+        if prefix is None or not torch.cuda.is_current_stream_capturing():
+            tops = torch.stack([t.abs().amax() for pair in kv for t in pair]).tolist()
         if prefix is None:
             per = -(-P // CACHE_PAGE)
-            tops = torch.stack([t.abs().amax() for pair in kv for t in pair]).tolist()
             caches = [kv4.Kv4Cache.empty(B * per, CACHE_PAGE, cfg.heads, cfg.head_dim, kv4.global_for(CACHE_MARGIN * kt),
                                          kv4.global_for(CACHE_MARGIN * vt), self.device)
                       for kt, vt in zip(tops[::2], tops[1::2])]
             table = torch.arange(B * per, dtype=torch.int32, device=self.device).view(B, per)
             prefix = Prefix([], P, P, caches, table, torch.full((B,), P, dtype=torch.int32, device=self.device))
+        elif tops is not None:
+            room = [g for c in prefix.caches for g in (c.k_global, c.v_global)]
+            over = max(t / (kv4.FP4_TOP * kv4.E4M3_TOP * g) for t, g in zip(tops, room))
+            if over > 1:
+                warnings.warn(f"build_prefix(into=...): this prompt's largest key or value is {over:.2f} times what the kept "
+                              "4-bit prefix's scales reach and saturates; a new prefix would hold it", stacklevel=4)
         first = torch.zeros_like(prefix.lengths)
         for cache, (k, v) in zip(prefix.caches, kv):
             kv4.write(cache, prefix.table, first, k.view(B * P, cfg.heads, cfg.head_dim),
