@@ -27,6 +27,7 @@ struct AttnParams {
   int items;             // few rows: upper bound of work items of a cache head; many rows: the grid's blocks
   int slots;             // blocks that the GPU holds at a time, per cache head (0: no sequence is split)
   int min_tiles;         // a work item has at least this many tiles of keys
+  float* carry;          // many rows: sums taken out of TMEM on the way, or null where no row block is that long
   float* part;           // partial results; few rows: [heads][items][rows][dim], many: [2 items][dim / 4][rows][4]; then
                          // their rows' (maximum, sum) pairs
 };

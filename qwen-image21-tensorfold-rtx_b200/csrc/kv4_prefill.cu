@@ -65,6 +65,12 @@ enum Bar {
   KFULL = 0, KEMPTY = 2, VFULL = 4, VEMPTY = 6, SFULL = 8, QFULL = 10, PFULL = 12, ODONE = 16, IDLE = 18, GFULL = 20,
   GEMPTY = 24
 };
+// The tensor core adds to its fp32 accumulators by cutting off, not by rounding: a sum of values of one sign loses about
+// 6e-9 of itself for every key (0.16 % after 262144, 10 % after 16 million). So every kCarry tiles a share's accumulators and
+// row sums are added to their sums in memory, with rounding, and begin again at zero: 1e-4 is lost at most, a fifth of half a
+// step of fp16. 128 KB a block, which stay in L2; a kernel of its own where the table and the new rows have room for more
+// tiles (4.33 -> 4.49 ms for 2048 rows x 32 heads on 8 over 131072 keys; up to 128 tiles the test alone would cost 2 %).
+constexpr int kCarry = 128;
 constexpr int kSegs = 4;                 // row blocks' shares that the warps are told of ahead
 // Some waits last as long as a whole share does (64 million keys a second): the one for room to hand out another, and those
 // of warps that have nothing to do in it. A stall inside a share runs into one of its own waits and ends these as well.
@@ -381,7 +387,7 @@ __device__ bool find_place(const AttnParams& p, int cut, int64_t x, Place& w) {
   return false;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CARRY>
 __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_constant__ AttnParams p,
                                                                const __grid_constant__ CUtensorMap k_map,
                                                                const __grid_constant__ CUtensorMap v_map,
@@ -695,7 +701,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     if (advance()) {
       begin(0);
       for (int jj = 0, j = 0; ok; ++jj) {
-        const bool last = j + 1 == n, cached = j < nc, add = j > 0;
+        const bool last = j + 1 == n, cached = j < nc, add = CARRY ? (j & (kCarry - 1)) != 0 : j > 0;
         const int rows2 = both;
         // The next tile is looked for ahead of this one's last product, but only one share ahead: shares without tiles are
         // handed out behind this share's results (of four shares the block knows at a time), which wait for that product.
@@ -738,6 +744,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     const uint32_t lane = (uint32_t)(warp & 3) << 21;       // this warp's 32 TMEM lanes
     const uint32_t ts = tmem + lane + i * 128, to = tmem + lane + kColO + i * 128 + half * (D / 2);
     float* pair = reinterpret_cast<float*>(smem + S::kPair) + i * 256 + r;
+    // this thread's sums in memory, 4 columns kRows apart, and their base and row sum (seldom used: addresses found there)
+    auto carry_sums = [&]() {
+      return reinterpret_cast<float4*>(p.carry) + (blockIdx.x * (D / 4) + half * (D / 8)) * kRows + i * 128 + r;
+    };
+    auto carry_row = [&]() {
+      return reinterpret_cast<float2*>(p.carry + (int64_t)p.items * kRows * D) + (blockIdx.x * 2 + half) * kRows + i * 128 + r;
+    };
     bool ok = true;
     int turn = 0, sp = 0, op = 0;        // phases waited for: scores, accumulators
     // what this thread tells the row's other one, for what that one tells (two buffers in turn: one barrier is enough; both
@@ -750,6 +763,30 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       return p2[(half ^ 1) * 128];
     };
     const float plain = fmaxf(fabsf(p.scale_log2), 1e-30f); // a scale of 0: any small one (-inf * 0 would be NaN)
+    // In front of tile j: the sums so far to those in memory, in plain values. The accumulator begins again with this tile's
+    // products (until then it may still be rescaled).
+    auto carry = [&](int j, int nc, float m, float& l) {
+      ok = ok && warp_wait(bar + SFULL + i, sp & 1, p.err, kErrPrefill + 10);    // behind all products of the tiles so far
+      if (!ok) return;
+      tc_after();
+      float2* row_at = carry_row();
+      const float2 old = j > kCarry ? *row_at : make_float2(m, 0.0f);
+      const float keep = exp2_fast(old.x - m), unit = j <= nc ? p.c.v_global : 1.0f;
+      *row_at = make_float2(m, old.y * keep + l);
+      l = 0.0f;
+#pragma unroll 1
+      for (int k = 0; k < D / 2; k += 16) {
+        uint32_t o[16];
+        tmem_ld16(to + k, o);
+#pragma unroll
+        for (int x = 0; x < 16; x += 4) {
+          float4* at4 = carry_sums() + (k + x) / 4 * kRows;
+          const float4 y = j > kCarry ? *at4 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          *at4 = make_float4(y.x * keep + __uint_as_float(o[x]) * unit, y.y * keep + __uint_as_float(o[x + 1]) * unit,
+                             y.z * keep + __uint_as_float(o[x + 2]) * unit, y.w * keep + __uint_as_float(o[x + 3]) * unit);
+        }
+      }
+    };
     // The next share. Both warps of a row go on or neither does.
     int at = 0;
     auto next_share = [&]() -> const Seg* {
@@ -815,6 +852,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       // (a share's first scores, where this query tile had no rows in the one before)
       if (live) ok = ok && warp_wait(bar + SFULL + i, sp & 1, p.err, kErrPrefill + 10, kShareLimitNs);
       for (int j = 0; live && j < n; ++j) {
+        if (CARRY && (j & (kCarry - 1)) == 0 && j > 0) carry(j, nc, m, l);
         ok = ok && warp_wait(bar + SFULL + i, sp++ & 1, p.err, kErrPrefill + 10);
         if (!ok) {
           tell(0.0f);
@@ -905,6 +943,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       ++at;
       const Seg* next = next_share();
       if (next && is_live(next)) e = put_query(next, next->nc > 0);
+      const bool carried = CARRY && live && n > kCarry;
+      float keep = 0.0f;
+      if (carried) {
+        const float2 old = *carry_row();
+        keep = exp2_fast(old.x - m);
+        l += old.y * keep;
+      }
       if (live) {
         ok = ok && warp_wait(bar + ODONE + i, op++ & 1, p.err, kErrPrefill + 12);
         tc_after();
@@ -918,6 +963,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       const int hq = g->h * p.group + row % p.group;
       const int64_t to_row = (int64_t)g->slot * kRows + i * 128 + r;
       const float f = l == 0.0f ? 0.0f : part ? unit : unit / l;
+      keep *= f / unit;
 #pragma unroll 1
       for (int k = 0; k < D / 2; k += 16) {
         uint32_t o[16];
@@ -934,6 +980,11 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
             float y[8];
 #pragma unroll
             for (int z = 0; z < 8; ++z) y[z] = __uint_as_float(o[x + z]) * f;
+            if (carried) {
+              const float4 a = carry_sums()[(k + x) / 4 * kRows], b = carry_sums()[((k + x) / 4 + 1) * kRows];
+              y[0] += a.x * keep, y[1] += a.y * keep, y[2] += a.z * keep, y[3] += a.w * keep;
+              y[4] += b.x * keep, y[5] += b.y * keep, y[6] += b.z * keep, y[7] += b.w * keep;
+            }
             if (part) {
               float4* to4 = reinterpret_cast<float4*>(p.part) +
                             ((int64_t)g->slot * (D / 4) + (col + x) / 4) * kRows + i * 128 + r;
@@ -1053,7 +1104,7 @@ __global__ void __launch_bounds__(256, 4) join_many_kernel(const __grid_constant
 
 struct ManyPlan {
   int blocks, min_tiles, join_blocks;    // blocks: 256 at most (a thread each of a join block)
-  int64_t ws;
+  int64_t ws, carry;                     // carry: its place in the workspace, or 0
 };
 ManyPlan many_plan(int64_t dim, int64_t heads, int64_t B, int64_t max_keys, int64_t T, int64_t group, int sms) {
   ManyPlan f;
@@ -1062,15 +1113,18 @@ ManyPlan many_plan(int64_t dim, int64_t heads, int64_t B, int64_t max_keys, int6
   const int64_t most = std::max<int64_t>(1, tiles) * (T * group / kRows + B) * heads;      // never fewer than there are
   f.blocks = static_cast<int>(std::min<int64_t>(std::min(sms, 256), std::max(heads * B, (most + f.min_tiles - 1) / f.min_tiles)));
   f.join_blocks = static_cast<int>(std::min<int64_t>(4 * f.blocks, 64 * heads * (T * group / kRows + B)));
-  f.ws = 2LL * f.blocks * kRows * (dim + 2) * 4 + f.blocks * (int64_t)sizeof(Joint);
+  f.ws = (2LL * f.blocks * kRows * (dim + 2) * 4 + f.blocks * (int64_t)sizeof(Joint) + 15) / 16 * 16;
+  f.carry = tiles - kLead > kCarry ? f.ws : 0;
+  if (f.carry) f.ws += (int64_t)f.blocks * kRows * (dim + 4) * 4;
   return f;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CARRY>
 tfb_status launch_many(AttnParams& p, const ManyPlan& f, const DeviceInfo* di, cudaStream_t s) {
   static std::atomic<bool> ready[64];
+  const auto kernel = attn_many_kernel<T, D, CARRY>;
   if (!ready[di->device].load(std::memory_order_acquire)) {
-    TFB_CUDA(cudaFuncSetAttribute(attn_many_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
+    TFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
     ready[di->device].store(true, std::memory_order_release);
   }
   // maps of the new keys and values; rows or heads without a stride of their own (expanded ones) are copied by hand
@@ -1082,11 +1136,15 @@ tfb_status launch_many(AttnParams& p, const ManyPlan& f, const DeviceInfo* di, c
     if (st == TFB_OK) st = make_tmap_rows16(&maps[1], p.vn, D, hk, vs * 2, p.a.T, p.vn_st * 2, 64, kKeys);
     if (st != TFB_OK) return st;
   }
-  TFB_CUDA(launch_pdl(attn_many_kernel<T, D>, dim3(f.blocks), dim3(kThreadsP), Smem<D>::kBytes, s, p, maps[0], maps[1],
-                      mapped));
+  TFB_CUDA(launch_pdl(kernel, dim3(f.blocks), dim3(kThreadsP), Smem<D>::kBytes, s, p, maps[0], maps[1], mapped));
   if (f.blocks > 1)
     TFB_CUDA(launch_pdl(join_many_kernel<T, D>, dim3(f.join_blocks), dim3(256), 0, s, p));
   return TFB_OK;
+}
+template <typename T>
+tfb_status launch_many_t(AttnParams& p, const ManyPlan& f, int64_t dim, const DeviceInfo* di, cudaStream_t s) {
+  if (dim == 128) return f.carry ? launch_many<T, 128, true>(p, f, di, s) : launch_many<T, 128, false>(p, f, di, s);
+  return f.carry ? launch_many<T, 64, true>(p, f, di, s) : launch_many<T, 64, false>(p, f, di, s);
 }
 
 }  // namespace
@@ -1105,8 +1163,8 @@ tfb_status attn_many(AttnParams& p, int dtype, int64_t dim, const DeviceInfo* di
   p.items = f.blocks;
   p.min_tiles = f.min_tiles;
   p.part = static_cast<float*>(ws);
-  if (dtype == TFB_DT_F16) return dim == 128 ? launch_many<__half, 128>(p, f, di, s) : launch_many<__half, 64>(p, f, di, s);
-  return dim == 128 ? launch_many<__nv_bfloat16, 128>(p, f, di, s) : launch_many<__nv_bfloat16, 64>(p, f, di, s);
+  p.carry = f.carry ? p.part + f.carry / 4 : nullptr;
+  return dtype == TFB_DT_F16 ? launch_many_t<__half>(p, f, dim, di, s) : launch_many_t<__nv_bfloat16>(p, f, dim, di, s);
 }
 
 }  // namespace tfb

@@ -172,3 +172,70 @@ def test_strides_of_a_single_row_or_head_do_not_matter(dev):
     assert one.data_ptr() % 16 == 0 and one.stride(1) % 8
     assert torch.equal(K.rope_axes(one[None], None, ids.expand(5, 3).contiguous(), (16, 24, 24))[0],
                        K.rope_axes(one.contiguous()[None], None, ids.expand(5, 3).contiguous(), (16, 24, 24))[0])
+
+
+# A product's fp32 accumulator is not rounded but cut: taken as 4 units at most (2^-21 of the sum so far) for each addition of 16
+# keys, half of that over a sum that grows evenly. Sums begin again every 128 tiles of 128 keys: 1024 additions.
+CUT = 1024 * 2.0 ** -21 / 2
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_sums_of_one_sign(dev, dim, dtype):
+    """A million keys in one block's share, all values of one sign: the sums hold (without carrying, 0.7 % was lost). One page
+    serves all positions: the exact result is that of 256 keys."""
+    heads, rows, page, n = 148, 64, 256, 1 << 20
+    assert takes_many([n], [rows], (heads, heads), page)
+    cache, one_table, _ = make_cache(dev, [page], heads, dim, page, seed=91, spare=0)
+    v = (randn((page, heads, dim), 92, torch.float32) * 0.2 + 1).to(dev)
+    k = torch.empty_like(v)
+    kv4.read(cache, one_table, ints([0], dev), k, torch.empty_like(v))
+    kv4.write(cache, one_table, ints([0], dev), k, v)
+    kv4.read(cache, one_table, ints([0], dev), k, v)
+    q = randn((rows, heads, dim), 93, dtype)
+    table = torch.zeros((1, n // page), dtype=torch.int32, device=dev)
+    out, lse = kv4.attention(q.to(dev), cache, table, ints([n], dev), return_lse=True)
+    half = torch.finfo(dtype).eps / 2
+    ref, ref_lse, tol, tol_lse = attend64(q.double().numpy(), [(k.double().cpu().numpy(), v.double().cpu().numpy())], [rows],
+                                          dim ** -0.5, False, half_step=half)
+    err = np.abs(out.double().cpu().numpy() - ref)
+    tol += CUT * np.abs(ref)
+    assert (err <= tol).all(), f"worst {np.max(err / tol):.2f} of the bound"
+    # 8192 roundings of 2^-24 each between two carries' 64, half of that over an even sum
+    off = np.abs(lse.double().cpu().numpy() - (ref_lse + math.log(n // page)))
+    assert (off <= tol_lse + 128 * 2.0 ** -25 + 64 * 2.0 ** -24).all(), off.max()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,new,causal,fresh", [(16384, 300, False, True), (16384, 300, True, True), (16300, 300, False, True),
+                                                (16640, 100, True, True), (33000, 129, True, False), (100, 17000, False, True)])
+def test_sums_carried_over_cached_and_new_keys(dev, dtype, n, new, causal, fresh):
+    """Shares of more than 128 tiles: sums are carried in front of, at and behind the border between cached and new keys. As many
+    sequences (on the same pages, with the same rows) as leave row blocks whole; the first one's rows are compared, all are alike."""
+    heads, dim, page = 2, 64, 256
+    seqs = 74 if new < 1000 else 2
+    pages = -(-n // page)
+    assert takes_many([n] * seqs, [new] * seqs, (heads, heads), page)
+    cache, table, seq = make_cache(dev, [n], heads, dim, page, seed=95)
+    q, k, v = (randn((new, heads, dim), 96 + i, dtype) for i in range(3))
+    rep = lambda t: t.to(dev).repeat(seqs, 1, 1)   # noqa: E731
+    own = dict(k_new=rep(k), v_new=rep(v)) if fresh else {}
+    out, lse = kv4.attention(rep(q), cache, table.expand(seqs, pages).contiguous(), ints([n] * seqs, dev), causal=causal, return_lse=True,
+                             **own)
+    out, lse = out.view(seqs, new, heads, dim), lse.view(seqs, new, heads)
+    if new < 1000:
+        assert (out == out[:1]).all() and (lse == lse[:1]).all()
+    some = slice(None) if new < 1000 else slice(0, new, 211)                 # (not causal there: rows do not depend on one another)
+    half = torch.finfo(dtype).eps / 2
+    n64 = lambda t: t.double().numpy()   # noqa: E731
+    kc, vc = seq[0]
+    if new < 1000:
+        ref, ref_lse, tol, tol_lse = attend64(n64(q), seq, [new], dim ** -0.5, causal, *((n64(k), n64(v)) if fresh else ()), new_p=half,
+                                              half_step=half)
+    else:
+        both = [(np.concatenate([kc, n64(k)]), np.concatenate([vc, n64(v)]))]
+        ref, ref_lse, tol, tol_lse = attend64(n64(q[some]), both, [len(q[some])], dim ** -0.5, False, cached_p=half, half_step=half)
+    err = np.abs(out[0, some].double().cpu().numpy() - ref)
+    tol += CUT * np.abs(ref)
+    assert (err <= tol).all(), f"worst {np.max(err / tol):.2f} of the bound"
+    assert (np.abs(lse[0, some].double().cpu().numpy() - ref_lse) <= tol_lse + 192 * 2.0 ** -24).all()
