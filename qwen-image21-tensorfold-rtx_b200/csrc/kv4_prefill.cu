@@ -163,6 +163,14 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
+// Shared memory by 32-bit addresses: through generic pointers the operand warps' stores and the softmax warps' exchange took
+// twice the registers for addresses, and of 80 a thread there are none to spare. What the compiler put away and loaded again
+// for every tile cost up to 20 % where one query tile's chain is all there is (64 rows x 16000 keys x 64: 144 us; 123 so),
+// 6 % of the ragged prefill chunk.
+__device__ __forceinline__ void store_shared(uint32_t dst, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -527,13 +535,17 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     const bool val = warp >= 18;
     const int t = threadIdx.x & 63;                         // rows t and t + 64 of a cached tile
     const int full = val ? VFULL : KFULL, empty = val ? VEMPTY : KEMPTY;
-    uint8_t* ring = smem + (val ? S::kV : S::kK);
+    const uint32_t ring = smem_u32(smem) + (val ? S::kV : S::kK);
     const uint8_t* codes = val ? p.c.v_codes : p.c.k_codes;
     const uint8_t* scales = val ? p.c.v_sf : p.c.k_sf;
     constexpr int CW = D / 32;           // 16-byte pieces of a row's codes
     bool ok = true;
     int sent = -1, done = 0;             // the last tile that TMA was asked for; tiles of the shares so far
-    int made = 0;                        // tiles of all, at the end
+    // Copies in flight land before the block's shared memory goes away, also where an error elsewhere ended the shares or the
+    // products. (Of the last two of `made` tiles: a stage that has been filled again was empty before. No wait without an error.)
+    auto land = [&](int made) {
+      for (int j = max(max(sent - 1, made - 2), 0); j <= sent; ++j) bar_drain(bar + full + (j & 1), (j >> 1) & 1);
+    };
     const Seg* g;
     for (int s = 0; ok && (g = share(s)); ++s) {
       const int nc = g->nc, n = nc + g->nf, f0 = g->f0, tile0 = g->tile0, len = g->len, nq = g->nq, h = g->h;
@@ -574,9 +586,11 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       for (int j = 0; j < nc && ok; ++j) {
         const int jj = done + j, st = jj & 1;
         if (jj >= 2) ok = warp_wait(bar + empty + st, ((jj >> 1) & 1) ^ 1, p.err, kErrPrefill + 1);
-        made = ok ? jj + 1 : jj;
-        if (!ok) break;
-        uint8_t* tile = ring + st * S::kTileB;
+        if (!ok) {
+          land(jj);
+          break;
+        }
+        const uint32_t tile = ring + st * S::kTileB;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           uint32_t sp[D / 32];             // scale pairs
@@ -593,7 +607,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
             for (int k = 0; k < 4; ++k) {  // word: 8 values, chunk 4 i + k; two chunks a scale
               uint32_t o[4];
               e2m1x8_scaled(words[k], __byte_perm(sp[i], 0, k < 2 ? 0x1010 : 0x3232), o);
-              *reinterpret_cast<uint4*>(tile + tile_at<D>(x * 64 + t, 4 * i + k)) = make_uint4(o[0], o[1], o[2], o[3]);
+              store_shared(tile + tile_at<D>(x * 64 + t, 4 * i + k), o[0], o[1], o[2], o[3]);
             }
           }
         }
@@ -611,8 +625,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
         for (int j = nc; j < n && ok; ++j) {
           const int jj = done + j, st = jj & 1;
           if (jj >= 2) ok = warp_wait(bar + empty + st, ((jj >> 1) & 1) ^ 1, p.err, kErrPrefill + 4);
-          made = ok ? jj + 1 : jj;
-          if (!ok) break;
+          if (!ok) {
+            land(jj);
+            break;
+          }
           const int first = (f0 + j - nc) * kKeys;
           if (mapped && first + kKeys <= nq) {              // whole tiles by TMA: one thread's work
             if (warp & 1) {
@@ -621,7 +637,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
               bar_arrive_tx(bar + full + st, S::kTileB);
 #pragma unroll
               for (int x = 0; x < D / 64; ++x)
-                copy_tensor_3d(ring + st * S::kTileB + x * S::kHalf, val ? &v_map : &k_map, bar + full + st, x * 64, h,
+                copy_tensor_3d(smem + (val ? S::kV : S::kK) + st * S::kTileB + x * S::kHalf, val ? &v_map : &k_map, bar + full + st, x * 64, h,
                                static_cast<int>(lo) + first);
             }
             __syncwarp();
@@ -629,7 +645,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
             continue;
           }
           // the sequence's last rows, zeros behind them (what lies there may be anything)
-          const uint32_t tile = smem_u32(ring + st * S::kTileB);
+          const uint32_t tile = ring + st * S::kTileB;
           const int key0 = first + r0;
           const T* from = src + key0 * ld + c * 8;
 #pragma unroll 8
@@ -645,9 +661,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
       }
       done += n;
     }
-    // Copies in flight land before the block's shared memory goes away, also where an error elsewhere ended the shares or the
-    // products. (Of the last two tiles: a stage that has been filled again was empty before. No wait without an error.)
-    for (int j = max(max(sent - 1, made - 2), 0); j <= sent; ++j) bar_drain(bar + full + (j & 1), (j >> 1) & 1);
+    if (ok) land(done);
   } else if (warp == 20) {
     // ------------------------------------------------------------------------------------------------- products
     const uint32_t qb = smem_u32(smem + S::kQ), kb = smem_u32(smem + S::kK), vb = smem_u32(smem + S::kV);
@@ -743,7 +757,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     const int i = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127;
     const uint32_t lane = (uint32_t)(warp & 3) << 21;       // this warp's 32 TMEM lanes
     const uint32_t ts = tmem + lane + i * 128, to = tmem + lane + kColO + i * 128 + half * (D / 2);
-    float* pair = reinterpret_cast<float*>(smem + S::kPair) + i * 256 + r;
+    const uint32_t pair = smem_u32(smem) + S::kPair + (i * 256 + r) * 4;
     // this thread's sums in memory, 4 columns kRows apart, and their base and row sum (seldom used: addresses found there)
     auto carry_sums = [&]() {
       return reinterpret_cast<float4*>(p.carry) + (blockIdx.x * (D / 4) + half * (D / 8)) * kRows + i * 128 + r;
@@ -756,11 +770,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) attn_many_kernel(const __grid_co
     // what this thread tells the row's other one, for what that one tells (two buffers in turn: one barrier is enough; both
     // warps come here equally often, also where a wait has run out)
     auto tell = [&](float x) -> float {
-      float* p2 = pair + (turn & 1) * 512;
+      const uint32_t p2 = pair + (turn & 1) * 2048;
       ++turn;
-      p2[half * 128] = x;
+      float y;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(p2 + half * 512), "f"(x) : "memory");
       asm volatile("bar.sync %0, 64;" ::"r"(1 + i * 4 + (warp & 3)) : "memory");
-      return p2[(half ^ 1) * 128];
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(p2 + (half ^ 1) * 512) : "memory");
+      return y;
     };
     const float plain = fmaxf(fabsf(p.scale_log2), 1e-30f); // a scale of 0: any small one (-inf * 0 would be NaN)
     // In front of tile j: the sums so far to those in memory, in plain values. The accumulator begins again with this tile's
