@@ -7,13 +7,17 @@
 namespace tfb {
 namespace {
 
-// Which kernel: an estimate of both, in microseconds beyond what they have in common. The kernel for few rows takes 16 rows
-// at a time through the keys, at about 15000 (row block, key) steps a microsecond over the GPU and 200 keys' time to begin
-// each; the one for many takes 256 rows and 2.8 us for 128 keys on each of 148 SMs, and does not split a sequence below 4
-// tiles. Up to 8 rows the first one always runs: they fill one fragment of it. Over 204 measured pairs (2 to 768 sequences
-// x heads, 60 to 32000 keys, 16 to 512 rows a head) it is 1.0 % above the better one on average, 40 % at worst. Few / many
-// in us, 64 rows a head: 18 / 25 (8 sequences x heads, 4000 keys), 105 / 62 (96, 4000), 22 / 25 (2, 32000), 318 / 219
-// (64, 32000); 16 rows: 41 / 61 (96, 4000); 256 rows: 101 / 41 (24, 4000).
+// Which kernel: two scores to compare. They are not times (large calls take half to two thirds of them, small ones more): only
+// which is smaller was fitted. The kernel for few rows takes 16 rows at a time through the keys, (row block, key) steps over
+// the whole GPU and 200 keys' worth to begin each; the one for many takes 256 rows, tiles of 128 keys over a B200's 148 SMs,
+// and does not split a sequence below 4 tiles. Up to 8 rows the first one always runs: they fill one fragment of it. Over
+// 204 sizes (2 to 768 sequences x heads, 60 to 32000 keys, 16 to 512 rows a head) the rule was 1.0 % above the better one on
+// average. Few / many in us, 64 rows a head: 16 / 24 (8 sequences x heads, 4000 keys), 111 / 62 (96, 4000), 320 / 214
+// (64, 32000), and the wrong way round 21 / 25 (2, 32000); 16 rows: 41 / 59 (96, 4000); 256 rows: 99 / 39 (24, 4000).
+// The lengths are on the device, so the keys are those that the table has room for. A table that is far larger than what the
+// sequences hold is judged as if full: 1000 keys, 256 rows a head, 8 sequences x heads take 23 / 26, of which a table for 1024
+// keys gets the first and one for 131072 the second; 500 keys, 64 rows, 64 take 25 / 18, a table for 512 the first, one for
+// 32768 the second. The worst found: 1000 keys, 32 rows, 256, which gets the first of 63 / 42 from either table.
 bool few_rows(int64_t B, int64_t heads, int64_t max_keys, int64_t T, int64_t group) {
   const double rows = static_cast<double>(T) * group / B, keys = static_cast<double>(max_keys) + static_cast<double>(T) / B;
   const double pairs = static_cast<double>(B) * heads, tiles = ceil(keys / 128);

@@ -1,10 +1,11 @@
 // Attention of few query rows (decode steps, drafted tokens) over the 4-bit cache. Its floor is the cache's bytes, 9/16 of a
-// byte per value; what bounds it is how many instructions a value costs. At HBM's rate an SM has 6 cycles for the 256
-// values of a key and head; a key takes 20 warp instructions, most of them conversions and the shifts that bring their
-// bytes up, on the ALU pipe at one every two cycles (54 % busy, issue slots 58 %). Measured on one B200: 32 ragged
-// sequences of up to 16384 keys, 8 heads x 128: 83 us (3.8 TB/s, floor 48 us); one sequence of 262143 keys, 4 heads: 46 us
-// (3.3 TB/s, floor 23 us); one of 300 keys, 24 heads: 6.7 us. Tiles of 64 keys and 12 warps an SM: 16 warps on tiles of 32
-// or 48 keys took 95 us for the first (spilled registers, a tile's fixed costs), byte shifts by multiplications 97 us.
+// byte per value. At HBM's rate an SM has 6 cycles for the 256 values of a key and head; a key takes 20 warp instructions,
+// most of them conversions and the shifts that bring their bytes up, on the ALU pipe at one every two cycles. No pipe is full
+// (ALU 54 % busy, issue slots 58 %): what bounds it are those instructions' latencies at 12 warps an SM, which their registers
+// allow. Measured on one B200: 32 ragged sequences of up to 16384 keys, 8 heads x 128: 82 us (3.8 TB/s, floor 48 us); one
+// sequence of 262143 keys, 4 heads: 44 us (3.4 TB/s, floor 23 us); one of 300 keys, 24 heads: 6.8 us. Tiles of 64 keys: 16
+// warps on tiles of 32 or 48 keys took 95 us for the first (spilled registers, a tile's fixed costs), byte shifts by
+// multiplications 97 us.
 //
 // A work item is a run of 64-key tiles of one sequence and cache head and up to 8 * NT query rows (the heads of the group,
 // times the sequence's rows). Its four warps take the tiles in turn; each warp keeps a ring of two tiles in shared memory,
@@ -21,7 +22,9 @@
 // A value fragment pairs two keys of one channel: the nibbles of two keys' words are interleaved before the
 // conversion. P^T reaches the second product's layout by movmatrix. E2M1 times its E4M3 scale is exact in fp16; a
 // bf16 query row is brought to fp16 by a power of two (row_exponent). P is rounded to fp16 (by 2^-11 of it or 2^-32 of the
-// row's largest, see kHead), over new keys to q's type.
+// row's largest, see kHead), over new keys to q's type. The products cut off where they add to fp32: a sum of values of one
+// sign loses about 1e-8 of itself for every key of a warp, that is a quarter of an item's (5e-4, half a step of fp16, where an
+// item has 200000 keys).
 #include <math.h>
 
 #include <algorithm>
