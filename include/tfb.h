@@ -292,7 +292,8 @@ tfb_status tfb_kv4_read(const tfb_kv4_cache* c, const int32_t* table, int64_t ta
  * new rows up to i; without, the queries are the last rows of the cache, row i sees positions up to
  * lengths[b] - n_q + i. A row that sees nothing gives 0 (and lse = -inf); else a NaN or an infinity in a query row gives
  * NaN (out and lse). lse (nullable): fp32 [T, Hq], the natural logarithm of the row's sum. What lies behind a sequence's
- * length is not looked at; keys and values in front of it must be finite. ws: tfb_kv4_attention_ws bytes, 16-byte aligned, not shared by calls that may overlap. */
+ * length is not looked at; keys and values in front of it must be finite. A page outside [0, pages) in front of it is taken
+ * as the nearest one inside. ws: tfb_kv4_attention_ws bytes, 16-byte aligned, not shared by calls that may overlap. */
 int64_t tfb_kv4_attention_ws(const tfb_kv4_cache* c, int64_t B, int64_t max_pages, int64_t T, int64_t Hq);
 tfb_status tfb_kv4_attention(const tfb_kv4_cache* c, const int32_t* table, int64_t table_ld, int64_t B,
                              int64_t max_pages, const int32_t* lengths, const int32_t* cu, int64_t T, int64_t Hq,

@@ -1,9 +1,10 @@
 // Attention of many query rows over the 4-bit cache and the call's own keys / values. Its floor is the tensor cores' time,
 // 2048 cycles for a block's tile, which the exponentials between the two products match on the special function units
-// (16 a cycle and SM); what bounds it is the chain scores -> softmax -> probabilities -> products of a query tile, about
-// 4000 cycles long, of which the other query tile's hides a part, and at full load the board's power (1.8 GHz of 1.965).
-// Measured on one B200, over and over: 4096 rows x 24 heads over 256 cached and 4096 new keys 265 us (0.83 PFLOP/s, 51 %
-// of the measured bf16 rate); a ragged causal chunk over up to 9000 cached keys, 16 heads on 4, 209 us (0.84 PFLOP/s).
+// (16 a cycle and SM). What bounds it is the chain scores -> softmax -> probabilities -> products of a query tile, about
+// 4000 cycles long, of which the other query tile's hides a part: the tensor pipe is active 46 % of the time, no other pipe
+// more. Measured on one B200: 4096 rows x 24 heads over 256 cached and 4096 new keys 240 us (0.91 PFLOP/s, 56 % of the
+// measured bf16 rate), 270 us over and over, with the clock at the board's 1000 W down from 1.96 to 1.76 GHz; a ragged
+// causal chunk over up to 9000 cached keys, 16 heads on 4, 190 to 206 us (0.86 to 0.93 PFLOP/s).
 //
 // A block, one an SM, works through its share of the work (below), at any time on 256 query rows of one sequence and cache
 // head (row r: query r / group of the sequence, head r % group of the group, so that grouped heads share every tile of
@@ -221,7 +222,7 @@ __device__ __forceinline__ int tile_at(int r, int c) {
 //    order: what is at work at a time then has few heads, whose keys and values stay in L2 (24 heads x 16384 tokens).
 // A second kernel joins the parts of the row blocks that were cut (image step: 38 MB of them, about 9 us; their layout lets
 // neighbouring lanes, which hold neighbouring rows, store next to one another: row by row the parts took 8 us each).
-// Against a grid block for each row block (us): a ragged causal chunk, 240 row blocks of 16 to 71 tiles, 209 / 270; 256
+// Against a grid block for each row block (us, when the shares were built): a ragged causal chunk, 240 row blocks of 16 to 71 tiles, 209 / 270; 256
 // short sequences 128 / 210; 140 row blocks of 8 tiles 37 / 55; 148 of them 37 / 33 (the join finds nothing to do);
 // 4096 rows x 24 heads 265 / 272 (the SMs' clock falls from 1.89 to 1.8 GHz with their idle time gone).
 struct Seg {                 // what a grid block does of a row block

@@ -10,8 +10,9 @@
 // The work is bound by HBM: every value is read once and written once. A block takes a few tokens, computes their
 // cos / sin once into shared memory for all of their query and key heads, and a lane holds 8 values of a head.
 // Measured on one B200: 20790 tokens x 32 heads x 80 in fp16 39.7 us (5.4 TB/s); 4096 tokens x 48 heads x 128 in bf16
-// with the norm 22.0 us (4.6 TB/s; the norm's shuffles and products make it issue-bound); 8 tokens 2.8 us (a launch and
-// three loads that depend on one another).
+// with the norm 22.0 us (4.6 TB/s; latencies at 44 % of an SM's warps: the norm's shuffles and the loads of cos / sin from shared
+// memory hold a warp for 3.5 cycles an instruction, loads from memory for 2.5; issue slots 58 %); 8 tokens 2.8 us (a launch
+// and three loads that depend on one another).
 #include <math.h>
 #include <string.h>
 

@@ -138,7 +138,8 @@ def attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, lengths: to
     rows up to i; without them the queries are the last rows of the cache, row i of n sees positions up to
     lengths[b] - n + i. A row that sees nothing gives 0 (and lse -inf); else a NaN or an infinity in a query row
     gives NaN (and lse NaN). What lies behind a sequence's length is never looked at; keys and values in front of it must
-    be finite. Row tensors may have any strides with contiguous heads and 16-byte aligned rows.
+    be finite. Page numbers are taken into the pool: one outside of it (which ``write`` and ``read`` skip) reads the first
+    or last page's rows. Row tensors may have any strides with contiguous heads and 16-byte aligned rows.
     -> out [T, Hq, D], or (out, lse fp32 [T, Hq]: natural logarithm of the row's sum of exponentials)."""
     what = "kv4.attention"
     B, pages, ld = _batch(what, cache, table, lengths, cu)
