@@ -36,6 +36,7 @@ constexpr float kNoMax = -1e30f;   // a row's base before its first key: finite,
 // A row's powers are taken over a base kHead below its running maximum, which follows only a rise by more than 2^8: at their
 // rounding to 16 bits they reach 2^(kHead + 8) = 2^15 (fp16 holds 65504). So a probability keeps its 11 bits in fp16 down to
 // 2^-21 of the row's largest and is lost below 2^-32 of it, where 262144 keys together weigh 2^-14 (without the head 2^-7).
+// Exponents around 7 are rounded by 2^-22, about as much as the powers themselves: lse is off by up to 9e-7 where it is near 0.
 constexpr float kHead = 7.0f;
 constexpr float kLazy = 15.0f;     // the base stays while the maximum is at most this far above it
 
